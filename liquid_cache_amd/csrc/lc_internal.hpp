@@ -360,7 +360,7 @@ struct lc_ctx {
     // recently destroyed last; any replacement / eviction of an entry moves all of them to the graveyard.
     std::vector<lc_scan*> list_cache;
     std::atomic<uint64_t> evict_epoch{0};  // bumped (under `mu`, exclusively) whenever an entry is replaced or evicted
-    // The builder: ONE worker thread with its own (lowest-priority) stream runs the scan-level index builds off the query path.
+    // The builder: ONE worker thread with its own stream runs the scan-level index builds off the query path.
     std::mutex builder_mu;
     std::condition_variable builder_cv;
     std::deque<std::packaged_task<void()>> builder_q;

@@ -1191,7 +1191,6 @@ struct FbOffsets {  // what str_offset_pair reads of an entry
 #define LC_FB_ROWPAD 2u
 #endif
 template <bool kUni> constexpr uint32_t fb_row_words() { return (kUni ? 256u : uint32_t(kFlatBits)) + LC_FB_ROWPAD; }  // (+2: the store loop's bank spread)
-constexpr size_t kFbPoliteLds = 2048;  // extra dynamic LDS of a "polite" build: 2 x (81,152 + 80 + 2,048) > 160 KiB, one workgroup per CU
 template <bool kUni> constexpr size_t fb_lds_bytes() {
     // stage + per-code table (8 bytes) + value ranges + first items (entry index in the top bits) + per-code first | last | len
     return size_t(kFbWords) * fb_row_words<kUni>() * 8u + 256u * 8u + size_t(kFbValues) * 8u + size_t(kFbValues) * 4u + 256u * 4u;
@@ -1448,6 +1447,37 @@ __global__ __launch_bounds__(kFbThreads) __attribute__((amdgpu_num_sgpr(80))) vo
     }
 }
 
+// The workgroups of a build over `n_groups` groups of `tiles` tiles each.  A build on the builder thread (`background`) goes out in
+// pieces of kFbPiece workgroups, each waited for before the next is launched: all streams have the same priority, a process has
+// few hardware queues, and a query whose stream shares the builder's queue waits for what the builder has launched — the whole
+// build when that is one launch.  The pieces are whole groups; only the base addresses differ between them.  512 is one workgroup
+// in every slot of the device (256 CUs, two each).  Measured with scripts/query_during_build.py (COUNT(*) queries on one 100 M-row
+// table while another one's index is built; worst query on one stream / on eight in turn, build time on one / on eight):
+//   one launch  72-102 us / 2,680-2,840 us    3.5 / 2.85 ms        1,024  86-89 us / 144-159 us    4.9 / 4.5 ms
+//   8,192       83-84 us / 708-811 us         3.7 / 3.1 ms           512  75-92 us / 90-108 us     4.5-5.1 / 4.7-5.1 ms
+//   2,048       87-90 us / 125-248 us         4.2 / 4.2 ms
+// (median 23-26 us throughout, as on a quiet device; a query waits for the workgroups in flight, ~50 us each, on any queue).  With no
+// query beside it a build takes 4.4 ms in pieces of 512 and 2.85 ms in one launch.
+#ifndef LC_FB_PIECE
+#define LC_FB_PIECE 512
+#endif
+constexpr uint32_t kFbPiece = LC_FB_PIECE;
+template <bool kUni>
+lc_status launch_flat_build(const FlatBuildArgs& a, uint32_t tiles, uint32_t n_groups, bool background, hipStream_t stream) {
+    constexpr auto kernel = k_flat_build<kUni, !kUni && LC_FB_SLOTS != 0>;
+    LC_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(fb_lds_bytes<kUni>())));
+    const uint32_t step = background ? std::max(1u, kFbPiece / tiles) : n_groups;
+    for (uint32_t g0 = 0; g0 < n_groups; g0 += step) {
+        if (g0) LC_HIP(hipStreamSynchronize(stream));
+        FlatBuildArgs piece = a;
+        piece.groups += g0;
+        piece.slices += uint64_t(g0) * a.group_stride;
+        hipLaunchKernelGGL(kernel, dim3(tiles, std::min(step, n_groups - g0)), dim3(kFbThreads), fb_lds_bytes<kUni>(), stream, piece);
+        LC_HIP(hipGetLastError());
+    }
+    return LC_OK;
+}
+
 // Where index memory comes from.  The index of a whole column is gigabytes and is an allocation of its own; the index of a
 // scan over ONE row group (the reference's granularity: a reader per row group) is a few megabytes, and a host that works at
 // that granularity creates and drops hundreds of such scans: as allocations of their own those were a hipMalloc per build and a
@@ -1520,11 +1550,8 @@ bool index_reserve(lc_ctx* ctx, uint64_t bytes, bool allow_evict, int* why) {
 // signature words), their records, and the kFlatBits slices built from the dictionary values.  A scan whose index does not
 // fit (more than half of the free device memory) keeps k_like_lean.  Fills the flat fields of `lp` — the scan's pipeline when
 // the caller waits for the build, a stand-in that the evaluating thread merges later when the builder thread runs it.
-// `polite` (the builder thread's builds): the kernel runs with ONE workgroup per CU instead of two.  A workgroup is 16 waves and
-// two of them take every wave slot of a CU for the ~4 ms the build of a 100 M-row column lasts — measured: a query launched
-// while the build ran waited until it had finished (4.2 ms for a 30 us kernel).  With one per CU (a kilobyte more of dynamic LDS
-// makes the second one not fit) half of the slots stay free for the queries the build must not hold up.
-lc_status build_flat(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t stream, bool allow_evict = true, bool polite = false) {
+// `background`: the builder thread's builds (see launch_flat_build).
+lc_status build_flat(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t stream, bool allow_evict = true, bool background = false) {
     LC_PHASE("build_flat (all; builder thread when async)");
     lp->flat = false;
     lp->flat_tried = true;
@@ -1651,17 +1678,7 @@ lc_status build_flat(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t stre
     // (no memset: the tiles of a group cover every word of its slices, padding included)
     FlatBuildArgs ba{lp->d_groups, s->d_symtabs, lp->d_slices, flat_slice_stride(uint32_t(groups.size()), gw),
                      flat_group_stride(kFlatBits, gw)};
-    LC_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_flat_build<false, true>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                               int(fb_lds_bytes<false>() + kFbPoliteLds)));
-    LC_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_flat_build<false>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                               int(fb_lds_bytes<false>() + kFbPoliteLds)));
-    if (polite)
-        hipLaunchKernelGGL((k_flat_build<false, true>), dim3(gw / kFbWords, uint32_t(groups.size())), dim3(kFbThreads),
-                           fb_lds_bytes<false>() + kFbPoliteLds, stream, ba);
-    else
-        hipLaunchKernelGGL((k_flat_build<false, LC_FB_SLOTS != 0>), dim3(gw / kFbWords, uint32_t(groups.size())), dim3(kFbThreads),
-                           fb_lds_bytes<false>(), stream, ba);
-    LC_HIP(hipGetLastError());
+    if (const lc_status st = launch_flat_build<false>(ba, gw / kFbWords, uint32_t(groups.size()), background, stream); st != LC_OK) return st;
     if (ev1) LC_HIP(hipEventRecord(ev1, stream));
     LC_HIP(hipStreamSynchronize(stream));  // the vectors are locals
     float ms = 0;
@@ -1683,7 +1700,8 @@ lc_status build_flat(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t stre
 // dictionary value (0.98 GB and one more pass over the dictionaries for the 100 M-row URL column).  A value holds the byte b
 // exactly when its bit in slice b is set, so a 1-byte LIKE needs no walk: k_like_scanall<kUni> copies the entry's words of
 // ONE slice and maps the rows through the keys.
-lc_status build_unigram(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t stream, uint64_t** out_uni, double* out_ms) {
+lc_status build_unigram(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t stream, uint64_t** out_uni, double* out_ms,
+                        bool background = false) {
     *out_uni = nullptr;
     *out_ms = 0;
     if (!lp->flat || !lp->d_dst_word || lp->slice_words == 0) return LC_OK;
@@ -1706,9 +1724,7 @@ lc_status build_unigram(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t s
     if (ev0) LC_HIP(hipEventRecord(ev0, stream));
     FlatBuildArgs ba{lp->d_groups, s->d_symtabs, d_uni, flat_slice_stride(lp->n_group_slots, lp->group_words),
                      flat_group_stride(256u, lp->group_words)};
-    hipLaunchKernelGGL(k_flat_build<true>, dim3(lp->group_words / kFbWords, lp->n_group_slots), dim3(kFbThreads),
-                       fb_lds_bytes<true>(), stream, ba);
-    LC_HIP(hipGetLastError());
+    if (const lc_status st = launch_flat_build<true>(ba, lp->group_words / kFbWords, lp->n_group_slots, background, stream); st != LC_OK) return st;
     if (ev1) LC_HIP(hipEventRecord(ev1, stream));
     LC_HIP(hipStreamSynchronize(stream));
     float ms = 0;
@@ -2290,16 +2306,6 @@ uint64_t like_pipeline_bytes(const lc_scan* s, const StrPredHost& sp, bool with_
 // (byte_view_array/conversions.rs:353-355: at insert time).  The first attempt never evicts another scan's cached index; a scan
 // that was turned away for that reason tries again, with eviction, once it has served kEvictAfterEvals evaluations.
 // Caller holds s->mu.
-// -DLC_FB_POLITE=1: the builder thread's builds run ONE workgroup per CU (build_flat's `polite`).  That form was this round's
-// first answer to "a query launched during a build waited 4.2 ms for its 30 us kernel"; the answer that holds is the streams'
-// priorities — queries run on streams of the highest priority, the builder's has the lowest, and a build workgroup lives ~50 us,
-// so a query's workgroups take the next free slots.  Measured with scripts/query_during_build.py (COUNT(*) queries on one table
-// while another table's index is built, 8 ms windows): two workgroups per CU — queries median 23-26 us (quiet device: 23.4), max
-// 66-81 us, build kernel 4.0 ms; one per CU — median 28-38 us, max 46-64 us, build kernel 5.0 ms.  The full-occupancy build
-// disturbs the median less (it is over sooner) and the worst query by 20 us more: it is the default.
-#ifndef LC_FB_POLITE
-#define LC_FB_POLITE 0
-#endif
 static lc_status want_flat_index(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipStream_t stream) {
     if (!lp->eligible || lp->flat) return LC_OK;
     LC_PHASE("like: want_flat_index");
@@ -2329,7 +2335,7 @@ static lc_status want_flat_index(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, hipS
     lp->flat_job = builder_submit(ctx, [ctx, s, lp, pend, allow_evict, gate](hipStream_t st) {
         build_gate_pass(gate);
         try {
-            (void)build_flat(ctx, s, pend, st, allow_evict, LC_FB_POLITE != 0);
+            (void)build_flat(ctx, s, pend, st, allow_evict, true);
         } catch (...) {
             pend->flat = false;
         }
@@ -2352,7 +2358,7 @@ static lc_status want_unigram_index(lc_ctx* ctx, lc_scan* s, LikePipeline* lp, h
         uint64_t* u = nullptr;
         double ms = 0;
         try {
-            (void)build_unigram(ctx, s, lp, st, &u, &ms);
+            (void)build_unigram(ctx, s, lp, st, &u, &ms, true);
         } catch (...) {
         }
         lp->uni_pending = u;

@@ -169,13 +169,9 @@ hipStream_t stream_acquire(lc_ctx* ctx) {
         }
     }
     if (!s) {
-        // (the highest priority the device offers: the streams queries run on must not queue behind the builder's stream)
-        int lo = 0, hi = 0;
-        if (hipDeviceGetStreamPriorityRange(&lo, &hi) != hipSuccess || hipStreamCreateWithPriority(&s, hipStreamNonBlocking, hi) != hipSuccess) {
-            (void)hipGetLastError();
-            s = nullptr;
-        }
-        if (!s && hipStreamCreateWithFlags(&s, hipStreamNonBlocking) != hipSuccess) return nullptr;  // null stream as a fallback
+        // (the default priority, as the builder's stream has it: streams of different priorities must not be busy at once; what
+        // keeps a query from waiting for an index build is that builds go out in pieces, see launch_flat_build)
+        if (hipStreamCreateWithFlags(&s, hipStreamNonBlocking) != hipSuccess) return nullptr;  // null stream as a fallback
         std::lock_guard<std::mutex> g(ctx->pool_mu);
         ctx->all_streams.push_back(s);
     }
@@ -184,18 +180,16 @@ hipStream_t stream_acquire(lc_ctx* ctx) {
 }
 void stream_release(lc_ctx*, hipStream_t) {}  // (the stream stays bound to the thread)
 
-// ---- the builder: one worker thread per context with a stream of its own at the lowest priority the device offers.  It runs
+// ---- the builder: one worker thread per context with a stream of its own (of the default priority, like every stream).  It runs
 // what a query should not wait for — the scan-level LIKE index of a scan (k_flat_build: ~4 ms and 2 GB per 100 M-row column)
 // — the way the reference derives its prefilter outside the read path (at insert time, byte_view_array/conversions.rs:353-355).
 // Started on first use, drained and joined by lc_ctx_destroy.
 static void builder_main(lc_ctx* ctx) {
     (void)hipSetDevice(ctx->device);
-    int lo = 0, hi = 0;
     hipStream_t st = nullptr;
-    if (hipDeviceGetStreamPriorityRange(&lo, &hi) != hipSuccess ||
-        hipStreamCreateWithPriority(&st, hipStreamNonBlocking, lo) != hipSuccess) {
+    if (hipStreamCreateWithFlags(&st, hipStreamNonBlocking) != hipSuccess) {
         (void)hipGetLastError();
-        if (hipStreamCreateWithFlags(&st, hipStreamNonBlocking) != hipSuccess) st = nullptr;
+        st = nullptr;
     }
     {
         std::lock_guard<std::mutex> g(ctx->builder_mu);
@@ -3851,11 +3845,7 @@ lc_status lc_stream_create(lc_ctx* ctx, void** out_stream) {
     if (ctx->device < 0) return fail(LC_ERR_DEVICE, "host-only context: no HIP device (there is no CPU fallback)");
     LC_HIP(hipSetDevice(ctx->device));
     hipStream_t s = nullptr;
-    int lo = 0, hi = 0;  // (query streams take the highest priority: see stream_acquire)
-    if (hipDeviceGetStreamPriorityRange(&lo, &hi) != hipSuccess || hipStreamCreateWithPriority(&s, hipStreamNonBlocking, hi) != hipSuccess) {
-        (void)hipGetLastError();
-        LC_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
-    }
+    LC_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));  // (the default priority: see stream_acquire)
     *out_stream = s;
     return LC_OK;
     });

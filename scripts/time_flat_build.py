@@ -1,5 +1,5 @@
 """k_flat_build alone: build time of the scan-level index of a 100 M-row URL column, synchronous (LC_OPT_LIKE_INDEX_ASYNC = 0:
-two workgroups per CU) and on the builder thread (polite: one per CU), three builds each; COUNT(*) checked every time.
+one launch) and on the builder thread (in pieces), three builds each; COUNT(*) checked every time.
 usage: python scripts/time_flat_build.py [--rows N]"""
 import argparse
 import os
@@ -38,7 +38,7 @@ def main():
             want = got if want is None else want
             info = sc.info()
             print("%s build %d: %.2f ms, index %.2f GB, COUNT(*) %d (%s), answered by %s" % (
-                "builder thread (polite)" if mode else "synchronous", k, info.index_build_ms, info.index_bytes / 1e9, got,
+                "builder thread" if mode else "synchronous", k, info.index_build_ms, info.index_bytes / 1e9, got,
                 "ok" if got == want else "MISMATCH", N.LIKE_KERNEL_NAMES.get(int(info.last_like_kernel))), flush=True)
             sc.close()
     cache.close()

@@ -43,3 +43,9 @@ def test_device_code_writes_through_vector_stores_only():
     """Nothing writes through the scalar data cache: its lines are not coherent with the vector caches, and writing a wave's ballots
     that way took 1.75 times as long as v_writelane and a vector store (134 MB written: 223 against 127 us)."""
     assert matches(SCALAR_WRITE) == []
+
+
+def test_every_stream_has_the_default_priority():
+    """The index builder's stream and the streams of queries are busy at the same time; work on streams of different priorities
+    may wait for good."""
+    assert matches(r"StreamPriority|StreamCreateWithPriority|is_high_priority_stream|Stream\([^)]*\bpriority\s*=") == []
