@@ -1076,6 +1076,7 @@ def make_abi_communicator(cache, N, Communicator, rank, world, torch, dist, dry_
     sharing one GPU under LC_BENCH_TEST_BACKEND): the shared-memory test backend, which RCCL's refusal of duplicate devices
     makes necessary."""
     import threading
+    from liquid_cache_amd import sharding
     note = None
     comm = None
     ok = 1
@@ -1113,7 +1114,7 @@ def make_abi_communicator(cache, N, Communicator, rank, world, torch, dist, dry_
     except Exception as e:  # noqa: BLE001 — never lose the scaling run to this path
         ok, note = 0, "%s: %s" % (type(e).__name__, e)
     agreed = torch.tensor([ok], dtype=torch.int64, device="cuda")
-    dist.all_reduce(agreed, op=dist.ReduceOp.MIN)
+    sharding.all_reduce(agreed, op=dist.ReduceOp.MIN)
     if int(agreed.item()) == 1:
         return comm, "lc_comm (%s through the C ABI), known-answer all-reduce passed on every rank" % (
             "shared-memory test backend" if dry_run else "RCCL")
@@ -1775,6 +1776,7 @@ def run_tpch_q6(cache, lc, N, args, rank, world, batch0, threads, scaling, torch
     number for every N and equals numpy's).  A step = the three fused passes (ship-date pair, discount pair, quantity),
     every mask the selection of the next, COUNT(*) produced by the last kernel and summed over ranks by an 8-byte
     all-reduce that overlaps the next step."""
+    from liquid_cache_amd import sharding
     from liquid_cache_amd.sharding import PipelinedCountAllReduce
     t_stage = time.perf_counter()
     ids, expected = stage_q6_columns(cache, lc, N, args, args.rows, threads, batch0)
@@ -1818,7 +1820,7 @@ def run_tpch_q6(cache, lc, N, args, rank, world, batch0, threads, scaling, torch
     elapsed = time.perf_counter() - t0
     t = torch.tensor([elapsed], dtype=torch.float64, device="cuda")
     if world > 1:
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        sharding.all_reduce(t, op=dist.ReduceOp.MAX)
     elapsed = float(t.item())
     hits = int(reducer.last().item())
     # per-batch counts of the last pass == numpy's per batch; their sum over ranks == the fused COUNT(*)
@@ -1829,7 +1831,7 @@ def run_tpch_q6(cache, lc, N, args, rank, world, batch0, threads, scaling, torch
     assert got.tolist() == expected.tolist(), "device COUNT(*) per batch differs from numpy"
     sums = torch.tensor([int(expected.sum()), int(s_ship.rows)], dtype=torch.int64, device="cuda")
     if world > 1:
-        dist.all_reduce(sums, op=dist.ReduceOp.SUM)
+        sharding.all_reduce(sums, op=dist.ReduceOp.SUM)
     assert int(sums[0].item()) == hits, "fused COUNT(*) %d != numpy %d" % (hits, int(sums[0].item()))
     rows_all = int(sums[1].item())
     # kernel time of one chain on this rank (HIP events on the launch stream)
@@ -1915,7 +1917,8 @@ def main():
     if not torch.cuda.is_available():
         raise SystemExit("bench.py needs a HIP device: liquid_cache_amd has no CPU fallback")
     # LC_BENCH_TEST_BACKEND=gloo: dry run of the multi-rank code path on a box with ONE GPU (every rank on device 0, the
-    # collectives through gloo) — a test aid for the launcher / sharding / reporting logic, never a measurement
+    # collectives through gloo, which is given host copies) — a test aid for the launcher / sharding / reporting logic, never a
+    # measurement
     test_backend = os.environ.get("LC_BENCH_TEST_BACKEND")
     if test_backend:
         local_rank = 0
@@ -2018,6 +2021,7 @@ def main():
     t_stage += time.perf_counter() - t_rot
     # COUNT(*) partials: written by the predicate kernel itself (lc_scan_eval_count); two buffers so that the all-reduce
     # of step i (RCCL's own stream) overlaps the scan of step i+1
+    from liquid_cache_amd import sharding
     from liquid_cache_amd.sharding import (Communicator, PipelinedAbiCountAllReduce, PipelinedCountAllReduce,
                                            all_gather_mask_segments)
     comm = None
@@ -2032,7 +2036,7 @@ def main():
     words_per_rank = None
     if comm and args.exchange == "mask":
         wl = [torch.zeros(1, dtype=torch.int64, device="cuda") for _ in range(world)]
-        dist.all_gather(wl, torch.tensor([words], dtype=torch.int64, device="cuda"))
+        sharding.all_gather(wl, torch.tensor([words], dtype=torch.int64, device="cuda"))
         words_per_rank = [int(x.item()) for x in wl]
         gathered[0] = torch.zeros(max(sum(words_per_rank), 1), dtype=torch.int64, device="cuda")
 
@@ -2107,12 +2111,12 @@ def main():
     loop_launch_ms = ev_loop0.elapsed_time(ev_loop1) / max(args.steps * sps, 1)  # per scan, launch gaps of one stream included
     t = torch.tensor([elapsed], dtype=torch.float64, device="cuda")
     if world > 1:
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        sharding.all_reduce(t, op=dist.ReduceOp.MAX)
     elapsed = float(t.item())
     ms_per_step = elapsed / args.steps * 1e3
     rows_t = torch.tensor([scan.rows], dtype=torch.int64, device="cuda")
     if world > 1:
-        dist.all_reduce(rows_t, op=dist.ReduceOp.SUM)
+        sharding.all_reduce(rows_t, op=dist.ReduceOp.SUM)
     rows_all = int(rows_t.item())
     step_no[0] = 0  # COUNT(*) of table 0 (the one the CPU oracle checks), through the same call
     one_scan()
@@ -2126,7 +2130,7 @@ def main():
     local_hits = int(counts.sum(dtype=torch.int64).item())
     lh = torch.tensor([local_hits], dtype=torch.int64, device="cuda")
     if world > 1:
-        dist.all_reduce(lh, op=dist.ReduceOp.SUM)
+        sharding.all_reduce(lh, op=dist.ReduceOp.SUM)
     assert int(lh.item()) == hits, "fused COUNT(*) %d != sum of per-entry counts %d" % (hits, int(lh.item()))
     # the same for every column of the rotation (the timed loop scans them all): fused COUNT(*) == sum of per-entry counts
     rot_hits, rot_counts = [hits], [counts.cpu().numpy().astype(np.int64)]
@@ -2195,14 +2199,14 @@ def main():
     kt = torch.tensor([kernel_ms, -kernel_ms], dtype=torch.float64, device="cuda")
     exchange_us = None
     if world > 1:
-        dist.all_reduce(kt, op=dist.ReduceOp.MAX)
+        sharding.all_reduce(kt, op=dist.ReduceOp.MAX)
         xbuf = torch.zeros((), dtype=torch.int64, device="cuda")
         for _ in range(5):
-            dist.all_reduce(xbuf)
+            sharding.all_reduce(xbuf)
         torch.cuda.synchronize()
         tx = time.perf_counter()
         for _ in range(50):
-            dist.all_reduce(xbuf)
+            sharding.all_reduce(xbuf)
         torch.cuda.synchronize()
         exchange_us = (time.perf_counter() - tx) / 50 * 1e6
 

@@ -10,6 +10,8 @@ Exchange steps (torch.distributed; backend "nccl" is RCCL over xGMI on ROCm, "gl
   * COUNT(*)-style consumers: one 8-byte all-reduce of the per-rank hit counts;
   * mask consumers: all-gather of the per-rank mask segments (disjoint row ranges, word-aligned per entry, so the
     gathered buffers concatenate without bit shifting).
+gloo is given host memory only: a tensor of another device is copied to the host first and back afterwards (its collectives on
+device tensors may hang when several ranks share one GPU).
 """
 from __future__ import annotations
 
@@ -63,11 +65,40 @@ def rank_of_entry(entry_id: int, shards: Sequence[Sequence[int]]) -> int:
     raise KeyError(entry_id)
 
 
+def _through_host(t, group) -> bool:
+    import torch.distributed as dist
+    return t.device.type != "cpu" and dist.get_backend(group) == "gloo"
+
+
+def all_reduce(t, op=None, group=None):
+    """torch.distributed.all_reduce in place (default: the sum)."""
+    import torch.distributed as dist
+    op = dist.ReduceOp.SUM if op is None else op
+    if _through_host(t, group):
+        host = t.cpu()  # (waits for what the current stream has queued)
+        dist.all_reduce(host, op=op, group=group)
+        t.copy_(host)
+    else:
+        dist.all_reduce(t, op=op, group=group)
+    return t
+
+
+def all_gather(outs, t, group=None):
+    """torch.distributed.all_gather into the tensors of `outs`."""
+    import torch.distributed as dist
+    if not _through_host(t, group):
+        dist.all_gather(outs, t, group=group)
+        return outs
+    hosts = [o.cpu() for o in outs]
+    dist.all_gather(hosts, t.cpu(), group=group)
+    for o, h in zip(outs, hosts):
+        o.copy_(h)
+    return outs
+
+
 def all_reduce_count(local_count, group=None):
     """Sum of per-rank hit counts (torch tensor, in place); the exchange step of COUNT(*) queries."""
-    import torch.distributed as dist
-    dist.all_reduce(local_count, op=dist.ReduceOp.SUM, group=group)
-    return local_count
+    return all_reduce(local_count, group=group)
 
 
 def all_gather_mask_segments(local_words, group=None):
@@ -77,6 +108,8 @@ def all_gather_mask_segments(local_words, group=None):
     shard order (per-entry segments are 64-bit aligned)."""
     import torch
     import torch.distributed as dist
+    if _through_host(local_words, group):
+        return [g.to(local_words.device) for g in all_gather_mask_segments(local_words.cpu(), group)]
     world = dist.get_world_size(group)
     n = torch.tensor([local_words.numel()], dtype=torch.int64, device=local_words.device)
     sizes = [torch.zeros_like(n) for _ in range(world)]
@@ -94,11 +127,13 @@ class PipelinedCountAllReduce:
 
     Two count buffers alternate: step i reduces into buffer i & 1 and starts its all-reduce asynchronously (RCCL runs it
     on its own stream, after the kernels already queued on the current stream); step i + 2 waits for that all-reduce
-    (a stream-side wait) before it overwrites the buffer.  `drain()` waits for everything outstanding."""
+    (a stream-side wait) before it overwrites the buffer.  `drain()` waits for everything outstanding.  Counts of a device that
+    gloo exchanges are reduced before submit() returns."""
 
     def __init__(self, make_buffer, world_size: int, group=None):
         self.buffers = [make_buffer(), make_buffer()]
         self.pending = [None, None]
+        self.through_host = None  # (known at the first submit(): a question to the process group, asked once)
         self.world = world_size
         self.group = group
         self.steps = 0
@@ -117,6 +152,11 @@ class PipelinedCountAllReduce:
         """Start the all-reduce of the buffer handed out by the last acquire()."""
         if self.world > 1:
             import torch.distributed as dist
+            if self.through_host is None:
+                self.through_host = _through_host(self.buffers[0], self.group)
+            if self.through_host:
+                all_reduce(self.buffers[self._current], group=self.group)
+                return
             self.pending[self._current] = dist.all_reduce(self.buffers[self._current], op=dist.ReduceOp.SUM,
                                                           group=self.group, async_op=True)
 

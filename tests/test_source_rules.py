@@ -49,3 +49,10 @@ def test_every_stream_has_the_default_priority():
     """The index builder's stream and the streams of queries are busy at the same time; work on streams of different priorities
     may wait for good."""
     assert matches(r"StreamPriority|StreamCreateWithPriority|is_high_priority_stream|Stream\([^)]*\bpriority\s*=") == []
+
+
+def test_tensors_are_exchanged_through_the_sharding_module():
+    """torch.distributed's collectives on tensors are called in sharding.py alone, which gives gloo host memory only: its collectives
+    on device tensors may hang when several ranks share one GPU."""
+    calls = matches(r"\bdist\.(?:all_reduce|all_gather|all_to_all|reduce|broadcast|gather|scatter|send|recv|i(?:send|recv))\w*\(")
+    assert [c for c in calls if not c.startswith("liquid_cache_amd/sharding.py:") and "_object" not in c] == []
