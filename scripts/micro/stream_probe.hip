@@ -1,5 +1,5 @@
 // Streaming-read policy probe (round 6): which load shape / cache policy / grid reads N bytes ONCE fastest on gfx950?
-//   hipcc --offload-arch=gfx950 -O3 -o stream_probe scripts/micro/stream_probe.hip && ./stream_probe [bytes]
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o stream_probe scripts/micro/stream_probe.hip && ./stream_probe [bytes]
 // Variants: plain 16-byte loads with U loads in flight per lane, the same non-temporal, LDS-DMA (global_load_lds, 1 KiB per
 // wave-instruction) with aux = 0 / 2 (nt) and R pieces in flight per wave; grids of CUs x {1, 2, 4, 8} workgroups of 256.
 // Prints one line per variant: us per pass and TB/s.  A micro-benchmark, not part of any library.

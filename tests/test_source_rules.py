@@ -24,7 +24,7 @@ def matches(pattern):
         with open(path, encoding="utf-8", errors="replace") as f:
             for no, line in enumerate(f, 1):
                 if rx.search(line):
-                    out.append("%s:%d: %s" % (os.path.relpath(path, ROOT), no, line.strip()[:120]))
+                    out.append("%s:%d: %s" % (os.path.relpath(path, ROOT), no, line.strip()))
     return out
 
 
@@ -56,3 +56,17 @@ def test_tensors_are_exchanged_through_the_sharding_module():
     on device tensors may hang when several ranks share one GPU."""
     calls = matches(r"\bdist\.(?:all_reduce|all_gather|all_to_all|reduce|broadcast|gather|scatter|send|recv|i(?:send|recv))\w*\(")
     assert [c for c in calls if not c.startswith("liquid_cache_amd/sharding.py:") and "_object" not in c] == []
+
+
+def test_hip_code_is_compiled_without_packed_fp32():
+    """The packed FP32 instructions are off wherever HIP code is compiled (hipcc makes them by itself from ordinary float code) and
+    written nowhere by hand: some of their forms may give wrong results."""
+    off = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+    with open(os.path.join(ROOT, "liquid_cache_amd", "csrc", "Makefile"), encoding="utf-8") as f:
+        text = f.read()
+    assert re.search(r"^DEVFLAGS := " + off + "$", text, re.M)
+    compiles = [line for line in text.splitlines() if "$(HIPCC)" in line and " -c " in line]
+    assert compiles and all("$(DEVFLAGS)" in line for line in compiles), compiles
+    lines = [m for m in matches(r"hipcc --offload-arch") if "__graft_entry__" not in m and "_native.py" not in m]
+    assert [m for m in lines if "packed-fp32-ops" not in m] == []
+    assert matches(r"(?:\b|\\[nt])v_pk_(?:add|mul|fma)_f32") == []
