@@ -67,7 +67,10 @@ def rank_of_entry(entry_id: int, shards: Sequence[Sequence[int]]) -> int:
 
 def _through_host(t, group) -> bool:
     import torch.distributed as dist
-    return t.device.type != "cpu" and dist.get_backend(group) == "gloo"
+    if t.device.type == "cpu":
+        return False
+    backends = dict(b.split(":") for b in dist.get_backend_config(group).split(","))  # e.g. cpu:gloo,cuda:nccl
+    return backends.get(t.device.type, dist.get_backend(group)) == "gloo"
 
 
 def all_reduce(t, op=None, group=None):

@@ -82,3 +82,23 @@ def test_host_tensors_are_given_as_they_are(gloo):
     t = torch.tensor([8], dtype=torch.int64)
     assert sh.all_reduce_count(t) is t
     assert gloo == [("all_reduce", "cpu")] and t.tolist() == [8]
+
+
+@pytest.mark.parametrize("backend", ["gloo", "cpu:gloo,cuda:gloo"])
+def test_a_device_tensor_goes_through_the_host_however_the_backend_is_named(tmp_path, backend):
+    dist.init_process_group(backend, init_method="file://%s" % (tmp_path / "store"), rank=0, world_size=1)
+    try:
+        t = Elsewhere([4])
+        t.device = torch.device("cuda")
+        assert sh._through_host(t, None)
+        assert not sh._through_host(torch.tensor([4]), None)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_a_device_of_another_backend_takes_its_tensors_itself(monkeypatch):
+    monkeypatch.setattr(dist, "get_backend_config", lambda group=None: "cpu:gloo,cuda:nccl")
+    monkeypatch.setattr(dist, "get_backend", lambda group=None: "cpu:gloo,cuda:nccl")
+    t = Elsewhere([4])
+    t.device = torch.device("cuda")
+    assert not sh._through_host(t, None)
